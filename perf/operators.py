@@ -13,7 +13,6 @@ tokens, chunks of 3120, 7020 at 720 x 1248, a prompt of 347) and ``wide`` (hidde
 of 10800 tokens, 512 condition tokens). Activations are N(0, 1) with 0.5 % of their channels scaled by 20,
 weights N(0, 0.02), biases N(0, 0.01).
 """
-import functools
 import math
 import os
 import sys
@@ -27,7 +26,6 @@ DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
 MAX_FLOPS = 2 * 10800 * 5120 * 15360
 
 
-@functools.lru_cache(None)
 def _package():
     at = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "joyai-video-edit_amd")
     if at not in sys.path:
