@@ -24,6 +24,7 @@
 #include "joy_common.hpp"
 #include "joy_kernels.hpp"
 #include "mxfp4_common.hpp"
+#include "mxfp4_schedule.hpp"
 
 namespace joy {
 namespace {
@@ -140,13 +141,11 @@ __device__ __forceinline__ void run_tiles(const MxGemmArgs& g, const MxTilePlan&
   constexpr int NA = (BM + 127) / 128, NW = (BN + 127) / 128;  // 1 KB scale loads a workgroup and slab
   constexpr int W_OFF = BM * RB, SA_OFF = W_OFF + BN * RB, SW_OFF = SA_OFF + NA * 1024;
   constexpr int SLAB = SW_OFF + NW * 1024;
-  constexpr int kStores = FM * (kEpi == kGeluQuant ? (FN + 1) / 2 + (FN == 3 ? 3 : 1) : FN * 2);  // a wave and tile
+  constexpr MxTileCounts kCounts = {FM, FN, S, kEpi == kGeluQuant};
   constexpr int PITCH = kStagePitch;
   constexpr int FA = FN / 2;  // W units of a slab's first phase
-  // loads behind the ones that a slab's last phase waits for: A rows of the slabs from the next but one on to the one S
-  // ahead, W rows and scales of all of these but the last
-  constexpr int kAhead = (S - 1) * IA + (S - 2) * (IW + 1);
-  static_assert(SLAB == tiles_lds(FM, FN) && S >= 2 && kAhead + kStores < 64, "LDS, vmcnt range");
+  static_assert(IA == kCounts.a() && IW == kCounts.w(), "loads of a slab");
+  static_assert(SLAB == tiles_lds(FM, FN) && S >= 2 && kCounts.next_slab_first() < 64, "LDS, vmcnt range");
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -543,10 +542,16 @@ __device__ __forceinline__ void run_tiles(const MxGemmArgs& g, const MxTilePlan&
     // in a tile's first slab the last epilogue's stores lie behind those loads too (none before the first tile, whose
     // first two slabs have landed)
     aim();
-    slab_step(std::true_type{}, IC<kAhead + kStores>{}, n_next);
+    slab_step(std::true_type{}, IC<kCounts.next_slab_first()>{}, n_next);
     for (int k = 1; k < nk; ++k) {
       aim();
-      slab_step(std::false_type{}, IC<kAhead>{}, 0);
+      slab_step(std::false_type{}, IC<kCounts.next_slab()>{}, 0);
+    }
+    if constexpr (kCounts.side_waits()) {
+      if (nk == 1) {  // no wait since this tile's bias and gate were loaded covers them
+        wait_vmcnt<kCounts.side()>();
+        block_barrier();
+      }
     }
     epilogue(o.m0, o.n0);
     side_at = 2048 - side_at;
