@@ -159,26 +159,23 @@ __device__ __forceinline__ void run_tiles(const MxGemmArgs& g, const MxTilePlan&
       __builtin_amdgcn_make_buffer_rsrc((void*)g.gate, 0, kEpi == kResidual ? g.N * 2 : 0, 0x00020000);
   if (first >= count) return;
 
-  // ---- the stream of loads: tile lb, slab lk
+  // ---- the stream of loads
   __amdgpu_buffer_rsrc_t ars, wrs, srs;
   uint32_t oa[IA], ow[IW], os = 0;
-  int k_off = -RB, s_off;  // the slab's bytes into a row, and into the scales
   const int sidx = wave % (NA + NW);  // this wave's scale load (waves past the last repeat one: the same bytes)
   const bool s_is_a = sidx < NA;
   const uint32_t s_lds = s_is_a ? SA_OFF + sidx * 1024 : SW_OFF + (sidx - NA) * 1024;
   const int s_step = (int)(s_is_a ? g.slab_a : g.slab_b);
-  int lb = first, lk = 0;
-  s_off = -s_step;
+  MxLoadStream at = {first, RB, s_step};
   auto load_tile = [&](int b) {
     const MxOrigin o = tile_origin<BM, BN, kMainRows, kRest>(plan, b);
     const int64_t m0 = o.m0;
-    const int n0 = o.n0;
-    // (the last 192-column tile of MXFP4 output may lie behind N: no columns, no scales)
-    const int rows = (int)min((int64_t)BM, g.M - m0), cols = __builtin_amdgcn_readfirstlane(max(min(BN, g.N - n0), 0));
+    const int n0 = mx_load_column(o.n0, g.N);
+    const int rows = (int)min((int64_t)BM, g.M - m0), cols = min(BN, g.N - n0);
     ars = __builtin_amdgcn_make_buffer_rsrc((uint8_t*)g.A + m0 * Kb, 0, rows * Kb, 0x00020000);
     wrs = __builtin_amdgcn_make_buffer_rsrc((uint8_t*)g.W + (int64_t)n0 * Kb, 0, cols * Kb, 0x00020000);
     const uint8_t* sp = s_is_a ? (const uint8_t*)g.scales_a + m0 * 8 : (const uint8_t*)g.scales_b + (int64_t)n0 * 8;
-    const int64_t end = s_is_a || cols > 0 ? (int64_t)(nk - 1) * s_step + (s_is_a ? g.M - m0 : g.N - n0) * 8 : 0;
+    const int64_t end = (int64_t)(nk - 1) * s_step + (s_is_a ? g.M - m0 : g.N - n0) * 8;
     srs = __builtin_amdgcn_make_buffer_rsrc((uint8_t*)sp, 0, (int)end, 0x00020000);
     const int lrow = lane >> 3, lchunk = lane & 7;  // 8 rows a load
 #pragma unroll
@@ -195,24 +192,19 @@ __device__ __forceinline__ void run_tiles(const MxGemmArgs& g, const MxTilePlan&
   };
   // load number d of the slab's A rows, and of its W rows and (the last) scales
   // (the range check of a raw buffer includes the scalar offset)
-  auto load_a = [&](int d, uint32_t slab) { dma_buf16(slab + (wave * IA + d) * 1024, oa[d], ars, k_off); };
+  auto load_a = [&](int d, uint32_t slab) { dma_buf16(slab + (wave * IA + d) * 1024, oa[d], ars, at.k_off); };
   auto load_w = [&](int d, uint32_t slab) {
     if (d < IW)
-      dma_buf16(slab + W_OFF + (wave * IW + d) * 1024, ow[d], wrs, k_off);
+      dma_buf16(slab + W_OFF + (wave * IW + d) * 1024, ow[d], wrs, at.k_off);
     else
-      dma_buf16(slab + s_lds, os, srs, s_off);
+      dma_buf16(slab + s_lds, os, srs, at.s_off);
   };
   // before a slab's loads: on to the next tile after the last slab of one, and to loads that fetch nothing after the
   // last tile. Outside the slab's code, whose MFMAs stay in place only in one basic block
   auto aim = [&]() {
-    k_off += RB;
-    s_off += s_step;
-    if (lk++ == nk) {
-      lk = 1;
-      k_off = s_off = 0;
-      lb += P;
-      if (lb < count) {
-        load_tile(lb);
+    if (at.next(nk, P, count, RB, s_step)) {
+      if (at.tile < count) {
+        load_tile(at.tile);
       } else {
         ars = wrs = srs = __builtin_amdgcn_make_buffer_rsrc((uint8_t*)g.A, 0, 0, 0x00020000);
       }
@@ -519,9 +511,9 @@ __device__ __forceinline__ void run_tiles(const MxGemmArgs& g, const MxTilePlan&
   };
 
   auto column_of = [&](int b) { return b < count ? tile_origin<BM, BN, kMainRows, kRest>(plan, b).n0 : 0; };
-  load_tile(lb);
-  load_side(column_of(lb), 0);
-  int n_next = column_of(lb + P);
+  load_tile(first);
+  load_side(column_of(first), 0);
+  int n_next = column_of(first + P);
 #pragma unroll
   for (int s = 0; s < S; ++s) {
     aim();

@@ -31,4 +31,29 @@ struct MxTileCounts {
   constexpr bool side_waits() const { return next_slab_first() > ws() + stores() + a(); }
 };
 
+// The loads of a workgroup's tiles first, first + P, ... below count as one stream of slabs, nk a tile: next() goes on by
+// one and says whether the tile has changed. Past the last tile the stream goes on with slabs that fetch nothing, from an
+// empty buffer range at offset 0: only against a range that holds them are scalar offsets sure to count as inside or
+// outside (an unsigned range minus offset would wrap).
+struct MxLoadStream {
+  int tile, slab = 0;
+  int k_off;       // the slab's bytes into a row
+  unsigned s_off;  // and into the scales (a whole tile's may pass 2^31)
+
+  constexpr MxLoadStream(int first, int row_bytes, int slab_stride)
+      : tile(first), k_off(-row_bytes), s_off(0u - (unsigned)slab_stride) {}
+  constexpr bool next(int nk, int P, int count, int row_bytes, int slab_stride) {
+    k_off += row_bytes, s_off += (unsigned)slab_stride;
+    if (slab++ != nk) return false;
+    tile += P;
+    slab = tile < count ? 1 : nk;  // behind the last tile every slab is as its first
+    k_off = 0, s_off = 0;
+    return true;
+  }
+};
+
+// First column that the loads of a tile at column n0 take: column 0 where the tile lies behind N (the last 192-column tile
+// of MXFP4 output may), whose results are not stored, so that its range of W holds every offset too.
+constexpr int mx_load_column(int n0, int N) { return n0 < N ? n0 : 0; }
+
 }  // namespace joy

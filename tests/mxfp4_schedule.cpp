@@ -1,7 +1,8 @@
 // Replays what one wave of the MXFP4 tile kernel issues, waits for and reads, with the counts that the kernel waits with
 // (csrc/mxfp4_schedule.hpp): every read of LDS has to lie behind a wait for its load and a barrier, every load into LDS
 // behind a barrier that follows the last read of what it overwrites. The four waves do the same in step, each a share of
-// the loads, so that one wave's wait before a barrier is every wave's.
+// the loads, so that one wave's wait before a barrier is every wave's. And where the stream of loads is: on the slabs of
+// the workgroup's tiles in turn, behind the last one at offset 0, at no time past a range.
 //
 // No arguments: the replay. Arguments fm fn ring quant: the count that the kernel waits with before the epilogue of a
 // tile of one slab, -1 where no wait is needed there.
@@ -60,6 +61,19 @@ static bool replay(const joy::MxTileCounts& n, int nk, int tiles, bool residual)
   return w.ok;
 }
 
+static bool stream(int nk, int first, int P, int count, int slab_stride) {
+  joy::MxLoadStream at = {first, 128, slab_stride};
+  bool ok = true;
+  for (int t = first; t < count; t += P)
+    for (int k = 0; k < nk; ++k) {
+      ok &= at.next(nk, P, count, 128, slab_stride) == (k == 0 && t != first);
+      ok &= at.tile == t && at.k_off == 128 * k && at.s_off == (unsigned)slab_stride * (unsigned)k;
+    }
+  for (int i = 0; i < 4; ++i)  // a ring's slabs behind the last tile
+    ok &= at.next(nk, P, count, 128, slab_stride) && at.tile >= count && at.k_off == 0 && at.s_off == 0;
+  return ok;
+}
+
 int main(int argc, char** argv) {
   if (argc == 5) {
     const joy::MxTileCounts n = {atoi(argv[1]), atoi(argv[2]), atoi(argv[3]), atoi(argv[4]) != 0};
@@ -81,6 +95,21 @@ int main(int argc, char** argv) {
                   printf("64 x %d rows, 64 x %d columns, ring of %d, %s output, %d slabs, %d tiles\n", fm, fn, ring,
                          quant ? "MXFP4" : "16-bit", nk, tiles), ++bad;
         }
+  for (int nk = 1; nk <= 5; ++nk)
+    for (int first = 0; first < 3; ++first)
+      for (int P = 3; P <= 4; ++P)
+        for (int count = first + 1; count <= 9; ++count)
+          for (int stride : {8, 8 * 347, nk > 1 ? 0x7ffffff8 / (nk - 1) / 8 * 8 : 0x7ffffff8}) {  // the largest: 2^31 bytes in all
+            ++runs;
+            if (!stream(nk, first, P, count, stride))
+              printf("stream of %d slabs, tiles %d, %d, ... below %d\n", nk, first, first + P, count), ++bad;
+          }
+  for (int N = 32; N <= 2048; N += 32)
+    for (int n0 = 0; n0 < (N + 255) / 256 * 256; n0 += 192) {
+      ++runs;
+      const int c = joy::mx_load_column(n0, N);
+      if (c >= N || (n0 < N && c != n0)) printf("column %d of %d: loads from %d\n", n0, N, c), ++bad;
+    }
   printf("%d of %d\n", bad, runs);
   return bad != 0;
 }
