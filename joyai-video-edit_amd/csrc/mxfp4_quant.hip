@@ -229,7 +229,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void norm_mod_mxfp4_rows(NormModArg
   auto range = [](const void* p, int bytes) { return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, bytes, 0x00020000); };
   auto row_of = [&](const void* p, int64_t first) { return range((const char*)p + first * ESZ, N * ESZ); };
   const auto xr = row_of(a.x, row * a.x_stride), scr = row_of(a.scale, mb * a.N), shr = row_of(a.shift, mb * a.N);
-  Raw8<DT> raw[VPT], sc[VPT], sh[VPT], ga[kAffine ? VPT : 1], be[kAffine ? VPT : 1];
+  Raw8<DT> raw[VPT], sc[VPT], sh[VPT], ga[kAffine ? VPT : 1], be[kAffine && NORM == 0 ? VPT : 1];
 #pragma unroll
   for (int i = 0; i < VPT; ++i) raw[i].template load<kNt>(xr, t * 8, i * T * 8);
 #pragma unroll
@@ -238,11 +238,15 @@ __global__ __launch_bounds__(64 * kRowWaves) void norm_mod_mxfp4_rows(NormModArg
     sh[i].template load<0>(shr, t * 8, i * T * 8);
   }
   if constexpr (kAffine) {
-    const auto gr = row_of(a.gamma, 0), br = range(a.beta, a.beta && NORM == 0 ? N * ESZ : 0);
+    const auto gr = row_of(a.gamma, 0);
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      ga[i].template load<0>(gr, t * 8, i * T * 8);
-      be[i].template load<0>(br, t * 8, i * T * 8);
+    for (int i = 0; i < VPT; ++i) ga[i].template load<0>(gr, t * 8, i * T * 8);
+    if constexpr (NORM == 0) {
+      // without beta an empty range at scalar offset 0: zeros
+      const auto br = range(a.beta, a.beta ? N * ESZ : 0);
+      const int step = a.beta ? T * 8 : 0;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) be[i].template load<0>(br, t * 8, i * step);
     }
   }
   if (t < 2 * kRowWaves && (t & (kRowWaves - 1)) >= T >> 6) (&red[0][0])[t] = 0.f;  // waves that the workgroup lacks
@@ -286,9 +290,9 @@ __global__ __launch_bounds__(64 * kRowWaves) void norm_mod_mxfp4_rows(NormModArg
     sc[i].get(m);
     sh[i].get(add);
     if constexpr (kAffine) {
-      float g[8], b[8];
+      float g[8], b[8] = {};
       ga[i].get(g);
-      be[i].get(b);
+      if constexpr (NORM == 0) be[i].get(b);
 #pragma unroll
       for (int j = 0; j < 8; ++j) y[j] = __builtin_fmaf(__builtin_fmaf(x[i][j] * r, g[j], b[j]), 1.f + m[j], add[j]);
     } else {
