@@ -55,3 +55,36 @@ def test_single_slab_tiles(M, N, K, dtype, kernel):
         q2, s2 = room(M, N)
         jo.mxfp4_scaled_mm_gelu_tanh_quant(a, w, sa, sw, b, q2, s2)
         assert (host(q2) == host(q)).all() and (host(s2) == host(s)).all()
+
+
+@pytest.mark.parametrize("M,N,kernel", [(347, 2080, "tiles<true, {}, 1, 2, 0>"), (701, 4096, "tiles<true, {}, 2, 2, 0>"),
+                                        (347, 14400, "tiles<true, {}, 2, 3, 0>"), (347, 16384, "tiles<true, {}, 2, 4, 0>"),
+                                        (3121, 5120, "tiles<true, {}, 4, 4, 1>")])
+def test_tiles_on_operand_views(M, N, kernel):
+    """Rows from an odd one on of larger operands and outputs (scale bases at 8 of 16 bytes, slabs further apart than their
+    rows), a residual whose rows are apart: each result, and the rows around the outputs as they were."""
+    import joyomni_ops as jo
+    announce("mxfp4 tiles on views", M, N)
+    K = 544  # the last slab has one block
+    a, w, sa, sw, va, vw, bias, res, gate = problem(M + 9, N + 16, K, "bf16", M)
+    rows, cols = slice(5, 5 + M), slice(3, 3 + N)
+    a, sa, w, sw = a[rows], sa[:, rows], w[cols].t(), sw[:, cols]
+    b, g = bias[cols].to(DEV), gate[cols].to(DEV)
+    y, tol = sums(va[rows], vw[cols], bias[cols])
+    out, names = kernels_of(lambda: jo.mxfp4_scaled_mm(a, w, sa, sw, torch.bfloat16, b))
+    expect(names, kernel, 0)
+    check_rounded(out, y, tol, "bf16")
+    z, ztol = mx.gelu_tanh(y), gelu_tol(y, tol)
+    check_rounded(jo.mxfp4_scaled_mm_gelu_tanh(a, w, sa, sw, torch.bfloat16, b), z, ztol, "bf16")
+    r = res.to(DEV)[rows, 8: 8 + N]
+    assert r.stride(0) == N + 16
+    g64, r64 = gate[cols].double().numpy(), res[rows, 8: 8 + N].double().numpy()
+    out, names = kernels_of(lambda: jo.mxfp4_scaled_mm_gated_residual(a, w, sa, sw, r, g, b))
+    expect(names, kernel, 2)
+    check_rounded(out, r64 + y * g64, abs(g64) * tol + 2.0 ** -23 * (abs(r64) + abs(y * g64)), "bf16")
+    q, s = room(M + 4, N)
+    _, names = kernels_of(lambda: jo.mxfp4_scaled_mm_gelu_tanh_quant(a, w, sa, sw, b, q[1: 1 + M], s[:, 1: 1 + M]))
+    expect(names, kernel, 3)
+    check_mx(q[1: 1 + M], s[:, 1: 1 + M].contiguous(), z, ztol)
+    for t in (q[:1], q[1 + M:], s[:, :1], s[:, 1 + M:]):
+        assert (t == 0x5a).all()
