@@ -501,7 +501,8 @@ def mxfp4_scaled_mm_gelu_tanh(mat_a, mat_b, scales_a, scales_b, out_dtype, bias:
 def mxfp4_scaled_mm_gated_residual(mat_a, mat_b, scales_a, scales_b, residual, gate,
                                    bias: Optional[torch.Tensor] = None, inplace: bool = False):
     """residual + mxfp4_scaled_mm(...) * gate in one kernel, rounded once to the residual's dtype; gate [N].
-    ``inplace=True`` writes into ``residual`` (contiguous) and returns it."""
+    ``inplace=True`` writes into ``residual`` and returns it: contiguous and at a 16-byte aligned address (the
+    other form copies a residual that is not aligned; this one refuses it)."""
     if inplace:
         _ops.mxfp4_scaled_mm_gated_residual_(mat_a, mat_b, scales_a, scales_b, residual, gate, bias)
         return residual

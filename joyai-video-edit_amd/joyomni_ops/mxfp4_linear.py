@@ -95,7 +95,8 @@ class MxFp4Linear(nn.Module):
 
     def gemm_gated_residual(self, x_q: torch.Tensor, x_scale: torch.Tensor, residual: torch.Tensor,
                             gate: torch.Tensor, inplace: bool = False) -> torch.Tensor:
-        """residual + gemm(x_q, x_scale) * gate in the product's epilogue; residual [M, N]."""
+        """residual + gemm(x_q, x_scale) * gate in the product's epilogue; residual [M, N], in place contiguous
+        and 16-byte aligned."""
         assert not self.gelu_tanh, "the gated-residual epilogue has no GELU"
         assert residual.dtype == self.out_dtype, "residual dtype must be the output dtype"
         return mxfp4_scaled_mm_gated_residual(x_q, self.weight_q, x_scale, self.weight_scale, residual, gate,

@@ -88,3 +88,18 @@ def test_tiles_on_operand_views(M, N, kernel):
     check_mx(q[1: 1 + M], s[:, 1: 1 + M].contiguous(), z, ztol)
     for t in (q[:1], q[1 + M:], s[:, :1], s[:, 1 + M:]):
         assert (t == 0x5a).all()
+
+
+def test_inplace_residual_alignment():
+    """A contiguous residual at an odd address: copied out of place, refused in place and then as it was."""
+    import joyomni_ops as jo
+    M, N, K = 9, 64, 64
+    a, w, sa, sw, _, _, bias, res, gate = problem(M, N, K, "bf16", 1)
+    odd = torch.zeros(M * N + 1, dtype=torch.bfloat16, device=DEV)[1:].view(M, N)
+    odd.copy_(res)
+    args = (a, w.t(), sa, sw)
+    want = jo.mxfp4_scaled_mm_gated_residual(*args, res.to(DEV), gate.to(DEV), bias.to(DEV))
+    assert torch.equal(jo.mxfp4_scaled_mm_gated_residual(*args, odd, gate.to(DEV), bias.to(DEV)), want)
+    with pytest.raises(RuntimeError, match="16-byte aligned"):
+        jo.mxfp4_scaled_mm_gated_residual(*args, odd, gate.to(DEV), bias.to(DEV), inplace=True)
+    assert torch.equal(odd.cpu(), res)

@@ -195,3 +195,10 @@ def test_block_precision_argument():
     from joyomni_ops.dit_block import QuantizedDoubleStreamBlock
     with pytest.raises(ValueError, match="precision must be"):
         QuantizedDoubleStreamBlock(64, 1, 64, "cpu", torch.Generator(), precision="int4")
+
+
+def test_inplace_residual_alignment():
+    """In place, a residual that is not 16-byte aligned is refused (out of place the operator copies it)."""
+    at = ctypes.c_void_p(P[6].value + 8)
+    refused(product("residual", res=at, out=at), 2, "16-byte aligned")
+    assert "16-byte aligned" in jo.mxfp4_scaled_mm_gated_residual.__doc__
