@@ -100,9 +100,12 @@ __device__ __forceinline__ void interleave_reads() {
 // while other rows' elements past K are whatever follows them, under scale bytes that are 0 in both operands: 2^-254
 // times at most 36 is 0 in fp32.
 //
-// What bounds it: with many tiles a CU the power. 10800 x 5120 x 15360 takes 370 us (4.59 PFLOP/s) at 1.69 GHz with the
+// What bounds it: with many tiles a CU the power. 10800 x 5120 x 15360 takes 376 us (4.52 PFLOP/s) at 1.69 GHz with the
 // MFMAs 63 % busy, 297 us with zeros for data (a loop of these MFMAs on registers alone reaches 6.7). In one round of
-// tiles it is the operand bytes of a CU, 35 (from HBM) to 45 (from the last-level cache) bytes a ns.
+// tiles operands arrive at 35 (from HBM) to 45 (from the last-level cache) bytes a ns and CU, half of what L2 gives 128-
+// byte rows; why no faster has not been found. The 256 x 256 kernels spill 56 to 72 bytes: in a tile's first slab a
+// reloaded address waits for every load and store in flight, and addresses reloaded behind the epilogue's stores wait
+// for these, so that each tile drains the ring's loads once or twice. The smaller tiles have no scratch.
 //
 // A workgroup's tiles of one shape: run_tiles() for main tiles, then for the rest's smaller ones (MxTilePlan).
 struct MxTilePlan {
@@ -582,9 +585,10 @@ hipError_t launch_tiles(const MxGemmArgs& g, const MxTilePlan& p, hipStream_t st
 
 // Few rows: a workgroup takes 32 NU columns of 32 MU rows and its waves share K, slab after slab (wave w the slabs w,
 // w + W, ...), each with a ring of S slabs in LDS of its own, so that no barrier holds up the loads, which are what
-// these calls are bound by. The partial sums go through LDS and are added in the order of the waves. W from HBM,
-// against the tile kernels: 1 x 4096 x 12288 12.5 -> 8.4 us (3.2 TB/s), 64 x 5120 x 5120 16.3 -> 8.4, 64 x 13824 x
-// 5120 31 -> 17, 64 x 5120 x 13824 18 -> 14.7.
+// these calls are bound by. The partial sums go through LDS and are added in the order of the waves. W from HBM, calls in a
+// loop with the gaps between launches, against the tile kernels: 1 x 4096 x 12288 12.5 -> 8.4 us (3.2 TB/s), 64 x 5120 x
+// 5120 16.3 -> 8.4, 64 x 13824 x 5120 31 -> 17, 64 x 5120 x 13824 18 -> 14.7. The kernels alone, W from HBM and from the
+// last-level cache: 7.6 and 5.6, 8.3 and 6.1, 14.9 and 11.8, 13.4 (216 workgroups on 256 CUs) and 10.5.
 template <bool kBf16, int kEpi, int NU, int MU, int W, int S>
 __global__ __launch_bounds__(64 * W) void mxfp4_gemm_rows(MxGemmArgs g) {
   constexpr int RB = 128, kUnit = 32 * RB + 256;   // a unit's rows, then their scales
